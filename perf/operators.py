@@ -3,9 +3,7 @@ gradient norm with clipping, and the row selection that densification does on 8-
 
 Every operator has a plain form here (elementary torch operations) and the framework's call; `own` says which one `run`
 makes.  The tensors of a case are views of flat buffers, each starting at a multiple of 256 elements: the plain forms
-work on the whole buffers, the framework's calls on the list of views, and both return the buffers.  A training
-program keeps its optimizer from step to step: `prepare` makes it where the framework's calls are timed, from the
-same tensors that the plain form has.
+work on the whole buffers, the framework's calls on the list of views, and both return the buffers.
 """
 import math
 import os
@@ -172,7 +170,7 @@ def prepare(case, seed):
     normal = lambda: torch.randn(at // BLOCK, BLOCK, generator=g, device=dev)  # noqa: E731
     uniform = lambda: torch.rand(at // BLOCK, BLOCK, generator=g, device=dev)  # noqa: E731
     mask = inside.view(-1, BLOCK)
-    s = {"op": case["op"]}
+    s = {"op": case["op"], "inside": inside}
     # gradients spread over some orders of magnitude; what no view of the step saw has none
     spread = size * torch.exp(1.5 * normal())
     grad = normal() * spread * (uniform() < 0.7) * mask
@@ -183,10 +181,10 @@ def prepare(case, seed):
         value = normal() * mask
         s["param"] = value.to(kind).view(-1)
         s["params"] = view(s["param"])
+    if case["op"] == "clip":
+        s["max_norm"] = MAX_NORM
         for p, q in zip(s["params"], s["grads"]):
             p.grad = q
-        s["max_norm"] = MAX_NORM
-    if case["op"] == "clip":
         return s
     if case["op"] != "rows8":
         s["master"] = None if kind == torch.float32 else s["param"].float()
@@ -197,6 +195,7 @@ def prepare(case, seed):
         s["number"] = torch.cat([torch.full((_blocks(n),), i) for i, (n, _, _) in enumerate(t)]).to(dev)
         s["first"] = torch.cat([torch.arange(_blocks(n)) * BLOCK for n, _, _ in t]).view(-1, 1).to(dev)
         s["lr_blocks"] = torch.tensor(s["lrs"], dtype=torch.float64, device=dev)[s["number"]].view(-1, 1)
+        s["max_norm"] = MAX_NORM
         s["eps"] = 1e-15
     # moments as they are after some steps: rows that were never seen have none
     seen = (uniform() < 0.95) * mask
@@ -205,8 +204,8 @@ def prepare(case, seed):
     m, v = 0.3 * normal() * spread * seen, (spread * (0.3 + uniform())) ** 2 * seen
     if case["op"] == "adamw":
         s["m"], s["v"] = m.view(-1), v.view(-1)
-        s["moments"] = list(zip(view(s["m"]), view(s["v"])))
-        return _with_optimizer(s)
+        s["ms"], s["vs"] = view(s["m"]), view(s["v"])
+        return s
     (mc, ms), (rc, rs) = _nearest(m), _nearest(v.sqrt(), root=True)
     s["m"], s["r"], s["m_scale"], s["r_scale"] = mc.view(-1), rc.view(-1), ms.view(-1), rs.view(-1)
     block = lambda flat: [flat[a // BLOCK:a // BLOCK + _blocks(n)] for a, (n, _, _) in zip(starts, t)]  # noqa: E731
@@ -225,21 +224,6 @@ def prepare(case, seed):
                 fresh = torch.full((int(case["new"] * rows),), -1, dtype=torch.int64, device=dev)
                 picks[rows] = torch.cat([kept, fresh])
             s["index"].append(picks[rows])
-        return s
-    return _with_optimizer(s)
-
-
-def _with_optimizer(s):
-    if own:
-        optim = _optim()
-        s["optimizer"] = optim.AdamW([{"params": [p], "lr": lr} for p, lr in zip(s["params"], s["lrs"])], betas=BETAS,
-                                     eps=s["eps"], weight_decay=s["decay"], moment_bits=32 if s["op"] == "adamw" else 8,
-                                     max_grad_norm=s["max_norm"] if s["clip"] else None, seed=SEED)
-        names = (("exp_avg", "exp_avg_sq") if s["op"] == "adamw" else
-                 ("exp_avg", "exp_avg_root", "exp_avg_scale", "exp_avg_root_scale"))
-        for i, (p, m) in enumerate(zip(s["params"], s["moments"])):
-            s["optimizer"].state[p] = {"step": s["step"], **dict(zip(names, m))} | (
-                {} if s["masters"] is None else {"master": s["masters"][i]})
     return s
 
 
@@ -258,11 +242,17 @@ def run(s):
         return _clip(s)
     if s["op"] == "rows8":
         return _rows(s)
+    s["step"] += 1
     if own:
-        s["optimizer"].step()
-        found = s["optimizer"].grad_norm
+        optim = _optim()
+        found = optim.grad_norm(s["grads"], s["max_norm"]) if s["clip"] else None
+        how = dict(step=s["step"], lr=s["lrs"], betas=BETAS, eps=s["eps"], weight_decay=s["decay"],
+                   masters=s["masters"], clip=found)
+        if s["op"] == "adamw":
+            optim.adamw_(s["params"], s["grads"], s["ms"], s["vs"], **how)
+        else:
+            optim.adamw8_(s["params"], s["grads"], s["moments"], seed=SEED, **how)
     else:
-        s["step"] += 1
         found = _plain_step(s)
     return {k: s[k] for k in ("param", "master", "m", "v", "r", "m_scale", "r_scale") if s.get(k) is not None} | (
         {} if found is None else {"norm": found})
