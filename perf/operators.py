@@ -237,6 +237,23 @@ def _optim():
     return optim
 
 
+def _optimizer(s):
+    """The optimizer that a training program makes before its first step and keeps: of the case's tensors, as they
+    stand before the pass."""
+    moments = zip(s["ms"], s["vs"]) if s["op"] == "adamw" else s["moments"]
+    names = (("exp_avg", "exp_avg_sq") if s["op"] == "adamw" else
+             ("exp_avg", "exp_avg_root", "exp_avg_scale", "exp_avg_root_scale"))
+    for p, g in zip(s["params"], s["grads"]):
+        p.grad = g
+    opt = _optim().AdamW([{"params": [p], "lr": lr} for p, lr in zip(s["params"], s["lrs"])], betas=BETAS, eps=s["eps"],
+                         weight_decay=s["decay"], moment_bits=32 if s["op"] == "adamw" else 8,
+                         max_grad_norm=s["max_norm"] if s["clip"] else None, seed=SEED)
+    for i, (p, m) in enumerate(zip(s["params"], moments)):
+        opt.state[p] = {"step": s["step"] - 1, **dict(zip(names, m))} | (
+            {} if s["masters"] is None else {"master": s["masters"][i]})
+    return opt
+
+
 def run(s):
     if s["op"] == "clip":
         return _clip(s)
@@ -244,14 +261,10 @@ def run(s):
         return _rows(s)
     s["step"] += 1
     if own:
-        optim = _optim()
-        found = optim.grad_norm(s["grads"], s["max_norm"]) if s["clip"] else None
-        how = dict(step=s["step"], lr=s["lrs"], betas=BETAS, eps=s["eps"], weight_decay=s["decay"],
-                   masters=s["masters"], clip=found)
-        if s["op"] == "adamw":
-            optim.adamw_(s["params"], s["grads"], s["ms"], s["vs"], **how)
-        else:
-            optim.adamw8_(s["params"], s["grads"], s["moments"], seed=SEED, **how)
+        if "optimizer" not in s:
+            s["optimizer"] = _optimizer(s)
+        s["optimizer"].step()
+        found = s["optimizer"].grad_norm
     else:
         found = _plain_step(s)
     return {k: s[k] for k in ("param", "master", "m", "v", "r", "m_scale", "r_scale") if s.get(k) is not None} | (
