@@ -148,13 +148,28 @@ __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY;
 __device__ __forceinline__ void update_moments(float g, float& m, float& v, float& root, const AdamWConst& c) {
 #pragma clang fp contract(off)
     m = m + c.one_minus_b1 * (g - m);
-    v = c.b2 * v + c.one_minus_b2 * (g * g);
+    const float decayed = c.b2 * v;
+    v = decayed + c.one_minus_b2 * (g * g);
+    // |g| from 2^64 on: g g is beyond 32 bits, its share in v need not be
+    if (__builtin_expect(!is_finite(v), 0)) v = decayed + c.one_minus_b2 * g * g;
     root = sqrtf(v);
 }
 
-__device__ __forceinline__ void update(float& p, float g, float& m, float& v, float& root, const AdamWConst& c,
-                                       const AdamWScalars& s) {
-    update_moments(g, m, v, root, c);
+// The same of m and the root r of v, which 32 bits hold for every finite g: where its square is beyond them it is taken
+// of 2^-70 of both, which loses nothing (what is lost beside it is below 2^-100 of it)
+__device__ __forceinline__ void update_moments_root(float g, float& m, float& r, const AdamWConst& c) {
+#pragma clang fp contract(off)
+    m = m + c.one_minus_b1 * (g - m);
+    const float v = c.b2 * (r * r) + c.one_minus_b2 * (g * g);
+    const float small = r * 0x1p-70f;
+    r = sqrtf(v);
+    if (__builtin_expect(!is_finite(v), 0)) {
+        g = g * 0x1p-70f;
+        r = sqrtf(c.b2 * (small * small) + c.one_minus_b2 * (g * g)) * 0x1p70f;
+    }
+}
+
+__device__ __forceinline__ void update_parameter(float& p, float m, float root, const AdamWConst& c, const AdamWScalars& s) {
     // the reciprocal's error of one unit is the update's, not the moments'
     p = p * s.keep - s.step_size * (m * __builtin_amdgcn_rcpf(root * s.rbc2 + c.eps));
 }
@@ -183,7 +198,8 @@ __device__ __forceinline__ void adamw_scalar(const AdamWTensor& t, const AdamWCo
             const long long i = at + 256 * j;
             if (i >= hi) continue;
             float root;
-            update(P[j], gs * G[j], M[j], V[j], root, c, s);
+            update_moments(gs * G[j], M[j], V[j], root, c);
+            update_parameter(P[j], M[j], root, c, s);
             w[i] = P[j];
             if (PT != AW_F32) store_from_float(t.p, PT, i, P[j]);
             m[i] = M[j];
@@ -213,11 +229,15 @@ __device__ __forceinline__ void adamw_vectors(const AdamWTensor& t, const AdamWC
 #pragma unroll
     for (int j = 0; j < U; j++) {
         const float4 x = Vec4<GT>::get(G[j]);
-        float root;
-        update(P[j].x, gs * x.x, M[j].x, V[j].x, root, c, s);
-        update(P[j].y, gs * x.y, M[j].y, V[j].y, root, c, s);
-        update(P[j].z, gs * x.z, M[j].z, V[j].z, root, c, s);
-        update(P[j].w, gs * x.w, M[j].w, V[j].w, root, c, s);
+        float4 root;
+        update_moments(gs * x.x, M[j].x, V[j].x, root.x, c);
+        update_moments(gs * x.y, M[j].y, V[j].y, root.y, c);
+        update_moments(gs * x.z, M[j].z, V[j].z, root.z, c);
+        update_moments(gs * x.w, M[j].w, V[j].w, root.w, c);
+        update_parameter(P[j].x, M[j].x, root.x, c, s);
+        update_parameter(P[j].y, M[j].y, root.y, c, s);
+        update_parameter(P[j].z, M[j].z, root.z, c, s);
+        update_parameter(P[j].w, M[j].w, root.w, c, s);
         store_parameter<PT>(t.p, w + 256 * j, q + 256 * j, P[j]);
         store_once(m + 256 * j, M[j]);
         store_once(v + 256 * j, V[j]);
@@ -303,9 +323,10 @@ __device__ __forceinline__ void adamw8_scalar(const AdamWTensor& t, const AdamWC
             const long long i = at + 64 * j + __lane_id();
             M[j] = R[j] = 0.0f;
             if (i < hi) {
-                float V = square(decode(D[j]) * rscale);
+                R[j] = decode(D[j]) * rscale;
                 M[j] = decode(C[j]) * mscale;
-                update(P[j], gs * G[j], M[j], V, R[j], c, s);
+                update_moments_root(gs * G[j], M[j], R[j], c);
+                update_parameter(P[j], M[j], R[j], c, s);
                 w[i] = P[j];
                 if (PT != AW_F32) store_from_float(t.p, PT, i, P[j]);
             }
@@ -382,8 +403,8 @@ __device__ __forceinline__ void adamw8_vectors(const AdamWTensor& t, const AdamW
         R[j][3] = __builtin_amdgcn_cvt_f32_fp8((int)D[j], 3) * rscale;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            float V = square(R[j][e]);
-            update(p4[e], g4[e], M[j][e], V, R[j][e], c, s);
+            update_moments_root(g4[e], M[j][e], R[j][e], c);
+            update_parameter(p4[e], M[j][e], R[j][e], c, s);
             mtop = fmaxf(mtop, finite_abs(M[j][e]));
             rtop = fmaxf(rtop, finite_abs(R[j][e]));
         }

@@ -299,6 +299,50 @@ def test_extreme_gradients_in_8_bits(optim, size):
     assert bool(torch.isfinite(p).all())
 
 
+@pytest.mark.parametrize("size", (2e19, 4e20, 6e20, 3e38))
+@pytest.mark.parametrize("bits", (32, 8))
+def test_gradients_whose_squares_leave_32_bits(optim, bits, size):
+    """|g| from 2^64 on, whose square is no 32-bit number, though (1 - b2) g g or its root may be one.  In 8 bits the
+    root is what is held, and 32 bits hold it for every finite g; a v of 32 bits beyond them is infinite (as
+    torch's) and its parameter stands still.  An ordinary step follows: nothing becomes NaN."""
+    g = torch.Generator().manual_seed(1)
+    n = 700
+    x = torch.randn(n, generator=g)
+    x[5], x[300], x[699] = size, -size, size
+    big = torch.zeros(n, dtype=torch.bool)
+    big[[5, 300, 699]] = True
+    p = cuda(torch.zeros(n))
+    opt = optim.AdamW([p], lr=1e-3, moment_bits=bits, weight_decay=0.0, eps=1e-15)
+    zero = torch.zeros(n, dtype=torch.float64)
+    want = [zero, zero, zero]
+    for t in (1, 2):
+        p.grad = cuda(x)
+        (p2, m2, v2), (ep, em, ev) = orc.adamw(*(want[:1] + [x] + want[1:]), step=t, lr=1e-3, eps=1e-15)
+        opt.step()
+        st = opt.state[p]
+        if t == 1 and bits == 8:
+            um, ur = orc.draws(n, 0, 0, 1)
+            orc.check_codes(st["exp_avg"], st["exp_avg_scale"], m2, em, um)
+            r = v2.sqrt()
+            orc.check_codes(st["exp_avg_root"], st["exp_avg_root_scale"], r, 12 * orc.U * r, ur, root=True)
+        if bits == 32:
+            there = v2 < 2.0 ** 127
+            assert float(((orc.f64(st["exp_avg_sq"]) - v2).abs() - ev)[there].max()) <= 0
+            assert bool((orc.f64(st["exp_avg_sq"])[~there] == math.inf).all())
+            if t == 1:
+                assert float(((orc.f64(p) - p2).abs() - ep)[there].max()) <= 0
+                assert bool((p.cpu()[~there] == 0).all())
+        assert bool(torch.isfinite(p).all())
+        # |m| / sqrt(v) is at most 3.2 from the second step on; 8 bits change either by an eighth and more
+        assert float(p.abs().max()) <= 1e-3 * t * 8
+        want = [p2, m2, v2]
+        if bits == 32:  # what the kernel holds
+            want = [orc.f64(p), orc.f64(st["exp_avg"]), orc.f64(st["exp_avg_sq"])]
+        else:
+            assert bool(torch.isfinite(st["exp_avg_root"].float()).all()) and bool((st["exp_avg_root"].float().cpu()[big] > 0).all())
+        x = torch.randn(n, generator=g)
+
+
 def test_a_root_never_vanishes(optim):
     """Gradients over twelve orders of magnitude in one block, most of them 0 in a step: r = 0 only
     where there never was a gradient, so m / (sqrt(v) + eps) is never m / eps."""
