@@ -235,6 +235,7 @@ int gsr_adam_step_range(long long n, long long lo, long long hi, int nseg, const
  * count after this update, g = grad_scale * clip[1] * grad:
  *     p *= 1 - lr weight_decay;  m += (1 - beta1)(g - m);  v = beta2 v + (1 - beta2) g g;
  *     p -= lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * An eps above 0 counts as at least 2^-126.
  * Types: 0 float, 1 bfloat16, 2 IEEE half.  A 16-bit param has a float master that takes the
  * update; param becomes its rounding.
  * clip: null, or two floats on the device, (norm, coefficient): gsr_grad_norm's over these and other

@@ -1920,7 +1920,10 @@ int gsr_adamw_step(int count, const gsr_adamw_tensor* tensors, int moment_bits, 
 
     gsr::AdamWTable a;
     memset(&a, 0, sizeof(a));
-    a.call.c = gsr::AdamWConst{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, grad_scale};
+    // the least normal number: a reciprocal of less is infinite, and 0 / eps would be NaN.  Beside a root above
+    // 0, which is at least 2^-75, either is nothing
+    const float least = eps > 0.0 ? std::max((float)eps, 0x1p-126f) : 0.0f;
+    a.call.c = gsr::AdamWConst{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), least, grad_scale};
     a.call.scalars = scalars;
     a.call.clip = clip;
     // every tensor once, in as many tables as it takes

@@ -343,6 +343,20 @@ def test_gradients_whose_squares_leave_32_bits(optim, bits, size):
         x = torch.randn(n, generator=g)
 
 
+@pytest.mark.parametrize("bits", (32, 8))
+@pytest.mark.parametrize("eps", (1e-30, 1e-38, 1e-40, 1e-44, 1e-60))
+def test_the_least_eps_divides_nothing_by_nothing(optim, bits, eps):
+    """Elements that never had a gradient stay where they are for every eps above 0, however small: 0 / eps is 0."""
+    p = cuda(torch.ones(600))
+    x = torch.zeros(600)
+    x[::7] = 1.0
+    p.grad = cuda(x)
+    opt = optim.AdamW([p], lr=1e-3, eps=eps, weight_decay=0.0, moment_bits=bits)
+    opt.step()
+    got = p.cpu()
+    assert bool((got[x == 0] == 1).all()) and float((got[x != 0] - (1 - 1e-3)).abs().max()) <= 4 * orc.U
+
+
 def test_a_root_never_vanishes(optim):
     """Gradients over twelve orders of magnitude in one block, most of them 0 in a step: r = 0 only
     where there never was a gradient, so m / (sqrt(v) + eps) is never m / eps."""
