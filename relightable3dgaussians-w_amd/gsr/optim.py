@@ -14,6 +14,7 @@ GPU tensors only: there is no CPU path.
 """
 from __future__ import annotations
 
+import collections
 import contextlib
 import ctypes as C
 import math
@@ -388,6 +389,14 @@ def _same_constants(a, b) -> bool:
     return len(a) == len(b) and all(x[0] == y[0] and x[1] == y[1] for x, y in zip(a, b))
 
 
+class _Loaded:
+    """A state on its way through torch's load_state_dict, which would cast a dict's tensors to their parameter's
+    type."""
+
+    def __init__(self, state: dict):
+        self.state = state
+
+
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update (no amsgrad) over all parameters in a few launches.
 
@@ -433,6 +442,9 @@ class AdamW(torch.optim.Optimizer):
                 "seed": self.seed, "max_grad_norm": self.max_grad_norm, "grad_norm": None}
 
     def __setstate__(self, state):
+        if "state" in state:  # what load_state_dict hands over is unwrapped
+            state = {**state, "state": collections.defaultdict(dict, {
+                p: st.state if isinstance(st, _Loaded) else st for p, st in state["state"].items()})}
         super().__setstate__(state)
         for g in self.param_groups:  # a state of another optimizer may lack some
             for k, v in self.defaults.items():
@@ -647,17 +659,26 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """Takes this class's or torch.optim.Adam / AdamW's state, with moments in either width (they
         are converted to this optimizer's).  A weight decay is AdamW's, whatever the state is of."""
-        saved = {k: v for k, v in state_dict["state"].items()}
+        last = self.register_load_state_dict_pre_hook(AdamW._before_load)  # behind the program's own: it sees what they return
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            last.remove()
+
+    def _before_load(self, state_dict) -> Optional[dict]:
+        """state_dict with its states as this optimizer holds them.  All that can be refused is refused here, before
+        anything changes."""
+        saved, groups = state_dict["state"], state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            return None  # torch says what is wrong
         for st in saved.values():
             if "max_exp_avg_sq" in st:
                 raise ValueError("AdamW: an amsgrad state cannot be loaded")
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        ids = [i for g in groups for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
-        for g in state_dict["param_groups"]:  # all that can be refused first: a refused one changes nothing
+        for g in groups:
             self._check_group({**self.defaults, **g})
-        states = [(p, self._converted(p, saved[i])) for i, p in zip(ids, params) if saved.get(i)]
-        super().load_state_dict({**state_dict, "state": {}})
-        self.state.update(states)
+        return {**state_dict, "state": {i: _Loaded(self._converted(p, saved[i])) for i, p in zip(ids, params) if saved.get(i)}}
 
     def _converted(self, p, saved) -> dict:
         take = lambda t: torch.as_tensor(t).detach().to(p.device).clone()  # noqa: E731

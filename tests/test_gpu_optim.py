@@ -1090,6 +1090,35 @@ def test_bfloat16_states_survive_a_state_dict(optim):
         assert w == v if k == "step" else w.dtype == v.dtype and torch.equal(w, v)
 
 
+@pytest.mark.parametrize("bits", (32, 8))
+def test_hooks_around_load_state_dict_see_the_state(optim, bits):
+    """Hooks before a load get the state that is loaded, and what they return is; hooks behind it find it in place."""
+    p = torch.randn(300, device=DEV).bfloat16().requires_grad_()
+    p.grad = torch.randn(300, device=DEV).bfloat16()
+    opt = optim.AdamW([p], moment_bits=bits)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    other = optim.AdamW([p], moment_bits=bits)
+    seen = []
+
+    def before(o, sd):
+        seen.append(sorted(sd["state"]))
+        sd = dict(sd, state={0: dict(sd["state"][0], step=41)})
+        return sd
+    other.register_load_state_dict_pre_hook(before)
+    other.register_load_state_dict_post_hook(lambda o: seen.append(int(o.state[p]["step"])))
+    other.load_state_dict(saved)
+    assert seen == [[0], 41] and saved["state"][0]["step"] == 1
+    st = other.state[p]
+    assert st["master"].dtype == torch.float32 and torch.equal(st["master"], opt.state[p]["master"])
+    assert torch.equal(raw(st["exp_avg"]), raw(opt.state[p]["exp_avg"]))
+    other.step()
+    assert int(other.state[p]["step"]) == 42
+    with pytest.raises(ValueError):  # refused by torch: another number of parameters
+        other.load_state_dict(dict(saved, param_groups=[dict(saved["param_groups"][0], params=[0, 1])]))
+    assert int(other.state[p]["step"]) == 42
+
+
 # ---- nothing outside
 
 class Fenced:
