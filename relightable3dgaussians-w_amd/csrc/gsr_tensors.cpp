@@ -315,10 +315,12 @@ PyObject* gsr_tensors_moment_rows(PyObject* tensors, gsr_moment_rows_tensor* out
 //                            and with or without a gradient as words[WORDS] says (1, 0), WORDS + 2 a row
 //   state, keys, values:     the state's keys and dicts are these
 //   names, state_words:      and the dicts hold these tensors
-// If so a new list of the gradients (or None), with at[i] their addresses, and *plain whether each is
-// dense, on its parameter's device, as large and of the type words[WORDS + 1]; else None.
+// If so a new list of the gradients (or None), with at[i] their addresses, *plain whether each is
+// dense, on its parameter's device, as large and of the type words[WORDS + 1], and *written whether a 16-bit
+// parameter that has one is of another version than versions[i] (-1: any is right); else None.
 PyObject* gsr_tensors_current(PyObject* groups, PyObject* params, const long long* words, PyObject* state, PyObject* keys,
-                              PyObject* values, PyObject* names, const long long* state_words, long long* at, int* plain) {
+                              PyObject* values, PyObject* names, const long long* state_words, long long* at, int* plain,
+                              const long long* versions, int* written) {
     return guarded(
         [&]() -> PyObject* {
             const Py_ssize_t n = PyList_GET_SIZE(params);
@@ -343,6 +345,7 @@ PyObject* gsr_tensors_current(PyObject* groups, PyObject* params, const long lon
             PyObject* grads = PyList_New(n);
             if (grads == nullptr) return nullptr;
             *plain = 1;
+            *written = 0;
             for (i = 0; i < n; i++) {
                 const long long* w = words + (WORDS + 2) * i;
                 const at::Tensor& g = THPVariable_Unpack(PyList_GET_ITEM(params, i)).grad();
@@ -359,11 +362,27 @@ PyObject* gsr_tensors_current(PyObject* groups, PyObject* params, const long lon
                 long long d[WORDS];
                 describe(o, d);
                 at[i] = d[0];
+                if (o != Py_None && w[2] > 0 && versions[i] != -1 &&
+                    THPVariable_Unpack(PyList_GET_ITEM(params, i))._version() != versions[i])
+                    *written = 1;
                 if (o != Py_None && (d[1] != w[1] || d[2] != w[WORDS + 1] || d[3] != w[3] || !d[4])) *plain = 0;
             }
             return grads;
         },
         nullptr);
+}
+
+// out[places[i]]: the version of parameter i of a list, if it is one of 16 bits.  0, or -1
+int gsr_tensors_versions(PyObject* params, const int* places, long long* out) {
+    return guarded(
+        [&] {
+            for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); i++) {
+                const at::Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(params, i));
+                if (p.scalar_type() != at::kFloat) out[places[i]] = p._version();
+            }
+            return 0;
+        },
+        -1);
 }
 
 }  // extern "C"

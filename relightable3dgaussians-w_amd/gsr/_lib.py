@@ -186,8 +186,9 @@ def tensors():
                 L.gsr_tensors_written_overlap.argtypes = [vp, C.c_int, C.c_int]
                 L.gsr_tensors_moment_rows.argtypes = [o, vp]
                 L.gsr_tensors_moment_rows.restype = o
-                L.gsr_tensors_current.argtypes = [o, o, vp, o, o, o, o, vp, vp, C.POINTER(C.c_int)]
+                L.gsr_tensors_current.argtypes = [o, o, vp, o, o, o, o, vp, vp, C.POINTER(C.c_int), vp, C.POINTER(C.c_int)]
                 L.gsr_tensors_current.restype = o
+                L.gsr_tensors_versions.argtypes = [o, vp, vp]
                 _tensors = L
     return _tensors
 

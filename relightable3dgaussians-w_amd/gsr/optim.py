@@ -305,7 +305,8 @@ class _Plan:
         self.states = [opt.state[p] for p in self.params]
         desc = self.desc = np.zeros(len(members), STEP_DTYPE)
         self.at = desc.ctypes.data
-        places = np.array(self.places, np.int32)
+        places = self.places_table = np.array(self.places, np.int32)
+        self.halves = any(p.dtype != torch.float32 for p in self.params)
 
         def planned() -> bool:
             return not _lib.tensors().gsr_tensors_plan(self.params, self.states, _names(self.bits), self.bits, opt.capturable,
@@ -359,7 +360,8 @@ class _Plan:
 class _Seen:
     """The optimizer's tensors that the plans were made of, as gsr_tensors_current compares them."""
 
-    def __init__(self, opt: "AdamW", params: List[torch.Tensor], grads: List[Optional[torch.Tensor]]):
+    def __init__(self, opt: "AdamW", params: List[torch.Tensor], grads: List[Optional[torch.Tensor]], left=None):
+        """left: what AdamW._left_behind says."""
         T = _lib.tensors()
         self.params, self.keys, self.values = params, list(opt.state), list(opt.state.values())
         self.names = _names(opt.moment_bits)
@@ -372,7 +374,14 @@ class _Seen:
         self.words = np.concatenate([words, there[:, None].astype(np.int64), grad_words[:, 2:3]], 1)
         self.at = np.zeros(len(params), np.int64)  # the gradients' addresses
         self.plain = C.c_int(0)
-        self.rest = (self.names, self.state_words.ctypes.data, self.at.ctypes.data, C.byref(self.plain))
+        # the versions of 16-bit parameters when their masters were last theirs; -1: not known, -2: another tensor's
+        self.versions = np.full(len(params), -1, np.int64)
+        for i, p in enumerate(params if left else ()):
+            if p in left:
+                self.versions[i] = left[p][1] if left[p][0] == words[i, 0] else -2
+        self.written = C.c_int(0)
+        self.rest = (self.names, self.state_words.ctypes.data, self.at.ctypes.data, C.byref(self.plain),
+                     self.versions.ctypes.data, C.byref(self.written))
         self.words_at = self.words.ctypes.data
 
     def grads(self, opt: "AdamW") -> Optional[List[Optional[torch.Tensor]]]:
@@ -402,7 +411,8 @@ class AdamW(torch.optim.Optimizer):
 
     * Parameters: float32, bfloat16 or float16, contiguous, on GPUs; gradients in any of the three.
       A 16-bit parameter has a 32-bit ``master`` in its state, which takes the update; the parameter
-      becomes its rounding.
+      becomes its rounding.  Where the program writes the parameter (a loaded model, a clamp), the next
+      step goes on from what it wrote; masters_from_parameters() says which writes cannot be seen.
     * ``moment_bits`` 32: the state is ``step``, ``exp_avg``, ``exp_avg_sq`` as torch's.  8:
       ``exp_avg`` and ``exp_avg_root`` (sqrt of exp_avg_sq) are e4m3 codes with a float scale for
       each 256 elements (``exp_avg_scale``, ``exp_avg_root_scale``): 2 bytes of state per element
@@ -431,6 +441,7 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm: Optional[torch.Tensor] = None
         self._plans: Optional[List[_Plan]] = None
         self._seen: Optional[_Seen] = None
+        self._left = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     # fixed: the states and the tables are made for them
@@ -450,6 +461,8 @@ class AdamW(torch.optim.Optimizer):
             for k, v in self.defaults.items():
                 g.setdefault(k, v)
         self._plans = self._seen = None
+        # loaded or copied masters are their parameters' as they are now
+        self._left = {p: (p.data_ptr(), p._version) for p, st in self.state.items() if "master" in st}
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
@@ -501,7 +514,32 @@ class AdamW(torch.optim.Optimizer):
             st.update(exp_avg=torch.zeros(p.shape, device=dev), exp_avg_sq=torch.zeros(p.shape, device=dev))
         if p.dtype != torch.float32:
             st["master"] = p.detach().float()
+            self._left[p] = (p.data_ptr(), p._version)
         return st
+
+    def _left_behind(self) -> dict:
+        """Of 16-bit parameters whose masters were once made of them or written to them: the address and version that
+        they had then."""
+        seen = self._seen
+        if seen is not None:
+            for k in np.flatnonzero(seen.versions != -1):
+                self._left[seen.params[k]] = (int(seen.words[k, 0]) if seen.versions[k] != -2 else -1, int(seen.versions[k]))
+            seen.versions[:] = -1
+        return self._left
+
+    def _master_from(self, p) -> None:
+        with torch.no_grad():
+            w = self.state[p]["master"].view(p.shape)
+            w.copy_(torch.where(w.to(p.dtype) == p, w, p.float()))
+
+    def masters_from_parameters(self) -> None:
+        """Makes the 32-bit masters those of their 16-bit parameters: a master whose rounding is its parameter stays,
+        another becomes the parameter's value.  step() does so by itself for parameters that were written since
+        the last one (by their version counter or another p.data); call this after writing past the counter
+        (p.data.copy_(...), a kernel of another library) or between replays of a captured step()."""
+        for p, st in self.state.items():
+            if st.get("master") is not None:
+                self._master_from(p)
 
     def _check_state(self, p, st) -> None:
         """Raises what a state lacks of what p's step takes; makes a master that is missing."""
@@ -524,6 +562,7 @@ class AdamW(torch.optim.Optimizer):
                 if _capturing(p.device):  # every replay would begin with the captured master
                     raise RuntimeError("AdamW: take one step() before the capture: it makes the states")
                 st["master"] = p.detach().float()
+                self._left[p] = (p.data_ptr(), p._version)
             full.append(("master", st["master"]))
             used.append(st["master"])
         for name, t in full:
@@ -556,7 +595,8 @@ class AdamW(torch.optim.Optimizer):
         every = plans[0].desc if len(plans) == 1 else np.concatenate([plan.desc for plan in plans] or [np.zeros(0, STEP_DTYPE)])
         if _lib.tensors().gsr_tensors_written_overlap(every.ctypes.data, len(every), self.moment_bits):
             raise ValueError("AdamW: parameters or states share memory")
-        self._seen = _Seen(self, flat, grads)
+        self._seen = _Seen(self, flat, grads, self._left_behind())
+        self._left = {}
         self._rates = None
         self._plans = plans
 
@@ -612,6 +652,10 @@ class AdamW(torch.optim.Optimizer):
                                "captured one)")
         clip, max_norm = None, -1.0
         seen, held = self._seen, [grads]  # kept until the launches
+        if seen.written.value:
+            for p, g, version in zip(seen.params, grads, seen.versions):
+                if g is not None and version != -1 and p._version != version:
+                    self._master_from(p)
         for plan in plans:
             every = len(plan.places) == len(grads)
             if seen.plain.value:
@@ -653,6 +697,8 @@ class AdamW(torch.optim.Optimizer):
             plan.steps += 1
         # the kernel wrote through raw pointers: saved-tensor checks and caches see it
         torch.autograd.graph.increment_version(plan.params)
+        if plan.halves and not torch.cuda.is_current_stream_capturing():  # a capture steps nothing yet
+            _lib.tensors().gsr_tensors_versions(plan.params, plan.places_table.ctypes.data, self._seen.versions.ctypes.data)
 
     # ---- states from elsewhere, and rows that come and go
 
@@ -758,4 +804,4 @@ class AdamW(torch.optim.Optimizer):
             g["params"][at] = q
             if k in states:
                 self.state[q] = states[k]
-        self._plans = self._seen = None
+        self._plans = None

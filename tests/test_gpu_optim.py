@@ -874,6 +874,99 @@ def test_a_state_or_a_parameter_that_was_replaced_is_used(optim):
     assert float(((orc.f64(opt.state[p]["exp_avg"]) - m2).abs() - em).max()) <= 0
 
 
+@pytest.mark.parametrize("bits", (32, 8))
+@pytest.mark.parametrize("kind", ("bf16", "fp16"))
+def test_a_16_bit_parameter_that_the_program_writes_is_kept(optim, bits, kind):
+    """Weights that the program puts into a 16-bit parameter between steps (a loaded model, a clamp, an average, a new
+    p.data) are what the next step starts from; where the parameter is its master's rounding the master stays."""
+    writes = (lambda p, x: p.copy_(x), lambda p, x: p[:100].copy_(x[:100]), lambda p, x: p.clamp_(-0.5, 0.5),
+              lambda p, x: setattr(p, "data", x.clone()), lambda p, x: p.mul_(1.0))
+    for write in writes:
+        opt, params, _ = make(optim, [(300,), (40,)], kind, bits=bits, weight_decay=0.0)
+        opt.step()
+        p, st = params[0], opt.state[params[0]]
+        x = torch.randn(300, device=DEV).to(p.dtype)
+        master = st["master"].clone()
+        with torch.no_grad():
+            write(p, x)
+        want = torch.where(master.to(p.dtype) == p, master, p.float())
+        other = opt.state[params[1]]["master"].clone()
+        before = [(None, q.grad.cpu(), w.cpu()) for q, w in zip(params, (want, other))]
+        moments = [[t.clone() for t in (opt.state[q][k] for k in optim._names(bits)[:-2])] for q in params]
+        opt.step()
+        for k, (q, (_, g, w), m) in enumerate(zip(params, before, moments)):
+            if bits == 8:
+                m, v = orc.value(m[0], m[2]), orc.value(m[1], m[3]) ** 2
+            else:
+                m, v = (t.cpu().double() for t in m)
+            check(opt, [q], [(None, g, w, m, v)], bits, step=8, weight_decay=0.0, first=k)
+    # a parameter that had no gradient meanwhile, and one step without it
+    opt, params, _ = make(optim, [(300,), (40,)], kind, bits=bits, weight_decay=0.0)
+    opt.step()
+    p, g = params[0], params[0].grad
+    p.grad = None
+    with torch.no_grad():
+        p.fill_(2.0)
+    opt.step()
+    assert bool((p == 2).all())
+    p.grad = g
+    m = [opt.state[p][k].clone() for k in optim._names(bits)[:-2]]
+    m, v = (orc.value(m[0], m[2]), orc.value(m[1], m[3]) ** 2) if bits == 8 else (t.cpu().double() for t in m)
+    opt.step()
+    check(opt, [p], [(None, g.cpu(), torch.full((300,), 2.0), m, v)], bits, step=8, weight_decay=0.0)
+
+
+def test_a_loaded_master_stays_with_its_parameter(optim):
+    """The optimizer's state before the model's weights, or behind them: the masters' lower bits survive both; weights
+    of another model do not lose to the masters."""
+    p = torch.randn(300, device=DEV).bfloat16()
+    p.grad = torch.randn(300, device=DEV).bfloat16()
+    opt = optim.AdamW([p], lr=1e-4, weight_decay=0.0)
+    for _ in range(3):
+        opt.step()
+    saved, weights = copy.deepcopy(opt.state_dict()), p.clone()
+    opt.step()
+    want, wanted = opt.state[p]["master"].clone(), p.clone()
+    for first in (True, False):
+        q = torch.zeros_like(p)
+        q.grad = p.grad
+        twin = optim.AdamW([q])
+        if first:
+            twin.load_state_dict(saved)
+        with torch.no_grad():
+            q.copy_(weights)
+        if not first:
+            twin.load_state_dict(saved)
+        twin.step()
+        assert torch.equal(twin.state[q]["master"], want) and torch.equal(q, wanted)
+    twin.load_state_dict(saved)
+    with torch.no_grad():
+        q.fill_(8.0)
+    twin.step()
+    assert float((twin.state[q]["master"] - 8).abs().max()) <= 1e-3
+
+
+def test_masters_in_a_captured_step(optim):
+    """A parameter that is written before the capture, and between replays through masters_from_parameters()."""
+    p = torch.zeros(300, dtype=torch.bfloat16, device=DEV)
+    p.grad = torch.zeros_like(p)
+    opt = optim.AdamW([p], capturable=True, weight_decay=0.0)
+    opt.step()
+    p.fill_(2.0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for value in (2.0, 3.0, 4.0):
+        p.data.fill_(value)  # no version counter tells this
+        opt.masters_from_parameters()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((p == value).all()) and bool((opt.state[p]["master"] == value).all())
+    opt.step()
+    assert bool((p == 4).all())
+
+
 def test_norm_order_is_fixed(optim):
     g = [torch.randn(n, device=DEV) for n in (100000, 77, 300001)]
     a = optim.grad_norm(g)
