@@ -137,7 +137,7 @@ def moments8_encode(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor) -> Moments8
     if exp_avg.shape != exp_avg_sq.shape or exp_avg.device != exp_avg_sq.device:
         raise ValueError("moments8_encode: the moments differ in shape or device")
     m = moments8_empty(exp_avg.shape, exp_avg.device)
-    a, b = exp_avg.detach().contiguous(), exp_avg_sq.detach().contiguous()
+    a, b = _solid(exp_avg.detach()), _solid(exp_avg_sq.detach())
     with _on(a.device):
         _lib.check(_lib.lib().gsr_moments_encode(a.numel(), a.data_ptr(), b.data_ptr(), *map(_data_ptr, m),
                                                  _stream(a.device)), "gsr_moments_encode")

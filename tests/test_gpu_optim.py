@@ -992,6 +992,14 @@ def test_encode_and_decode(optim, n):
     assert torch.equal(again.exp_avg.float(), e.exp_avg.float())
 
 
+def test_encoding_negated_views(optim):
+    """A view whose memory holds its values' negatives is encoded as its values."""
+    m, v = torch.randn(600, device=DEV), torch.rand(600, device=DEV)
+    want = optim.moments8_encode(m, v)
+    got = optim.moments8_encode(torch._neg_view(-m), torch._neg_view(-v))
+    assert all(torch.equal(raw(x), raw(y)) for x, y in zip(got, want))
+
+
 def test_encode_what_is_not_finite(optim):
     m = torch.randn(600)
     v = m * m
