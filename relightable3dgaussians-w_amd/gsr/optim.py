@@ -758,11 +758,15 @@ class AdamW(torch.optim.Optimizer):
         if not len(old) == len(new) == len(index):
             raise ValueError(f"replace_rows: {len(old)} old and {len(new)} new parameters and {len(index)} indices")
         where = {id(p): (g, k) for g in self.param_groups for k, p in enumerate(g["params"])}
-        seen = set()
+        seen, taken = set(), set()
+        others = set(where) - set(map(id, old))
         for p, q, ix in zip(old, new, index):
             if id(p) not in where or id(p) in seen:
                 raise ValueError("replace_rows: a parameter is not the optimizer's, or is listed twice")
+            if id(q) in taken or id(q) in others:
+                raise ValueError("replace_rows: a new parameter is listed twice, or is another one of the optimizer's")
             seen.add(id(p))
+            taken.add(id(q))
             self._check_param(q)
             if p.dim() == 0 or q.shape[1:] != p.shape[1:] or q.dtype != p.dtype or q.device != p.device:
                 raise ValueError(f"replace_rows: {tuple(q.shape)} {q.dtype} cannot take the place of "
@@ -798,9 +802,10 @@ class AdamW(torch.optim.Optimizer):
                 if "master" in st:
                     states[k]["master"] = rows(st["master"], new[k].detach().float())
             states[k]["step"] = st["step"]
+        for p in old:
+            self.state.pop(p, None)
         for k, (p, q) in enumerate(zip(old, new)):
             g, at = where[id(p)]
-            self.state.pop(p, None)
             g["params"][at] = q
             if k in states:
                 self.state[q] = states[k]

@@ -1135,6 +1135,20 @@ def test_replace_rows(optim, bits, kind):
     opt.step()
 
 
+def test_replace_rows_takes_each_parameter_once(optim):
+    """A new parameter that is listed twice, or is another one of the optimizer's, is refused and nothing changes."""
+    opt, params, _ = make(optim, [(10, 3), (10, 3)])
+    ix = torch.arange(10, device=DEV)
+    q = torch.zeros(10, 3, device=DEV)
+    for old, new in ((params, [q, q]), (params[:1], [params[1]])):
+        with pytest.raises(ValueError, match="replace_rows"):
+            opt.replace_rows(old, new, [ix] * len(old))
+        assert [g["params"][0] is p for g, p in zip(opt.param_groups, params)] == [True, True]
+        assert all(p in opt.state for p in params)
+    opt.replace_rows(params, params, [ix, ix.flip(0)])  # in their own places: other rows' moments
+    opt.step()
+
+
 @pytest.mark.parametrize("bits", (32, 8))
 def test_state_dicts(optim, bits):
     """Into this optimizer from torch's Adam, from moments of either width, and through copies."""
