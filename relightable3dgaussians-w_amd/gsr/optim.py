@@ -728,25 +728,29 @@ class AdamW(torch.optim.Optimizer):
 
     def _converted(self, p, saved) -> dict:
         take = lambda t: torch.as_tensor(t).detach().to(p.device).clone()  # noqa: E731
+        alike = lambda t: take(t).reshape(p.shape).contiguous()  # noqa: E731
         step = int(saved["step"])
         st = {"step": torch.full((), step, dtype=torch.int64, device=p.device) if self.capturable else step}
         sizes = {k: torch.as_tensor(saved[k]).numel() for k in ("exp_avg", "exp_avg_root", "exp_avg_sq", "master") if k in saved}
         if set(sizes.values()) != {p.numel()}:
             raise ValueError(f"AdamW: a state of {sizes} elements cannot be loaded for {tuple(p.shape)}")
         if "exp_avg_root" in saved:
-            m = Moments8(*(take(saved[k]) for k in Moments8._fields))
+            if any(k not in saved for k in Moments8._fields):
+                raise ValueError(f"AdamW: a state of 8-bit moments has {Moments8._fields}, got {tuple(saved)}")
+            m = _check_moments8([alike(saved[k]) for k in Moments8._fields[:2]] +
+                                [take(saved[k]).contiguous() for k in Moments8._fields[2:]], "AdamW: state", p.numel())
             if self.moment_bits == 8:
                 st.update(m._asdict())
             else:
                 st["exp_avg"], st["exp_avg_sq"] = moments8_decode(m)
         else:
-            m, v = (take(saved[k]).float().contiguous() for k in ("exp_avg", "exp_avg_sq"))
+            m, v = (alike(saved[k]).float() for k in ("exp_avg", "exp_avg_sq"))
             if self.moment_bits == 8:
                 st.update(moments8_encode(m, v)._asdict())
             else:
                 st.update(exp_avg=m, exp_avg_sq=v)
         if p.dtype != torch.float32:
-            st["master"] = take(saved["master"]).float() if "master" in saved else p.detach().float()
+            st["master"] = alike(saved["master"]).float() if "master" in saved else p.detach().float()
         return st
 
     def replace_rows(self, old: Sequence[torch.Tensor], new: Sequence[torch.Tensor],
@@ -781,7 +785,8 @@ class AdamW(torch.optim.Optimizer):
             for k in held:
                 byd.setdefault(old[k].device, []).append(k)
             for ks in byd.values():
-                rows = moments8_rows([[self.state[old[k]][f] for f in Moments8._fields] for k in ks],
+                rows = moments8_rows([[t.view(old[k].shape) if t.dtype == CODE else t for t in
+                                       (self.state[old[k]][f] for f in Moments8._fields)] for k in ks],
                                      [index[k].contiguous() for k in ks])
                 for k, m in zip(ks, rows):
                     states[k] = m._asdict()

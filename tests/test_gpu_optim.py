@@ -1234,6 +1234,37 @@ def test_hooks_around_load_state_dict_see_the_state(optim, bits):
     assert int(other.state[p]["step"]) == 42
 
 
+@pytest.mark.parametrize("bits", (32, 8))
+def test_states_of_other_layouts_are_loaded_as_the_parameters(optim, bits):
+    """Codes, moments and masters that were saved flat or transposed are laid out as their parameter; scales that do
+    not fit are refused before anything changes."""
+    p = torch.randn(40, 15, device=DEV).bfloat16()
+    p.grad = torch.randn(40, 15, device=DEV).bfloat16()
+    opt = optim.AdamW([p], moment_bits=bits)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    st = saved["state"][0]
+    for k in ("exp_avg", "exp_avg_root", "master"):
+        if k in st:
+            st[k] = st[k].t().contiguous().t() if k == "master" else st[k].reshape(-1)
+    other = optim.AdamW([p], moment_bits=bits)
+    other.load_state_dict(saved)
+    for k, t in opt.state[p].items():
+        if k != "step":
+            assert torch.equal(raw(other.state[p][k]), raw(t)) and other.state[p][k].shape == t.shape, k
+    if bits == 8:
+        ix = torch.tensor([3, -1, 39], device=DEV)
+        a, b = (optim.moments8_rows([[o.state[p][k] for k in optim.Moments8._fields]], [ix])[0] for o in (opt, other))
+        assert all(torch.equal(raw(x), raw(y)) for x, y in zip(a, b))
+        st["exp_avg_scale"] = st["exp_avg_scale"][:-1]
+        was = dict(other.state[p])
+        for o in (other, optim.AdamW([p])):
+            with pytest.raises(ValueError):
+                o.load_state_dict(saved)
+        assert all(other.state[p][k] is v for k, v in was.items())
+    other.step()
+
+
 # ---- nothing outside
 
 class Fenced:
