@@ -401,6 +401,46 @@ def test_the_expected_code_is_the_value(optim):
     assert float(r.std()) > 0
 
 
+def test_many_steps_of_8_bits_against_32(optim):
+    """2500 steps on the same stationary gradients with moments in 8 and in 32 bits (b2 = 0.999, c = 0.001, scales of
+    elements equal).  A root r that was rounded last step is a code, so this step it is off one by d = c / 2 |g^2 / v - 1|
+    of itself and, its block's scale moving likewise, by the difference of two such, E = c / 2 * 4 / pi; rounding
+    it up or down by a step s adds a variance of d s, and s is r / 16 to r / 8: S = 4e-5 to 8e-5 r^2 a step.
+    E[r] is kept and E[r^2] grows by S, which v forgets with c: v is too large by S / c, 4 to 8 %; r's deviation
+    decays by b2 a step, so its variance is S / (1 - b2^2): 14 to 20 %.  m is rounded at a random place of its step:
+    s^2 / 6 / (1 - 0.81), at most 12 % of m.  The update is off by both, at most 24 %; parts of a block far below its
+    largest value are held more coarsely and are not measured here.  Means over 2^16 elements: 4 % on top for
+    what is drawn, the 1 % by which E[1 / r] is more than 1 / E[r] and r's own spread (1.6 %)."""
+    n = 1 << 16
+    g = torch.Generator(device=DEV).manual_seed(11)
+    made = []
+    for bits in (32, 8):
+        p = torch.zeros(n, device=DEV)
+        made.append((p, optim.AdamW([p], lr=1.0, weight_decay=0.0, eps=1e-15, moment_bits=bits)))
+    total, moved = 0.0, None
+    for t in range(2500):
+        x = torch.randn(n, generator=g, device=DEV)
+        for p, opt in made:
+            p.zero_()  # the update alone
+            p.grad = x
+            opt.step()
+        if t >= 2000 and t % 50 == 0:
+            a, b = made[0][0].double(), made[1][0].double()
+            total += float(((a - b).norm() / a.norm())) / 10
+            moved = (a, b)
+    st = made[1][1].state[made[1][0]]
+    v = optim.moments8_decode([st[k] for k in optim.Moments8._fields])[1].double()
+    ratio = v / made[0][1].state[made[0][0]]["exp_avg_sq"].double()
+    assert 1.0 <= float(ratio.mean()) <= 1.08 + 0.04
+    root = ratio.sqrt()
+    assert 0.10 <= float(root.std()) <= 0.20 + 0.04
+    assert abs(float(root.mean()) - 1) <= 0.04 + 0.01
+    assert total <= 0.24 + 0.04
+    # the signs, and the sizes on average, are the exact update's
+    a, b = moved
+    assert abs(float((a * b).sum() / (a * a).sum()) - 1) <= 0.05
+
+
 def test_against_torch_over_steps(optim):
     """The reference's optimizer: one group per attribute, Adam with eps 1e-15 (gaussian_model.py:
     259-274), over 20 steps: the two round differently, by about U of a step's size each time."""
