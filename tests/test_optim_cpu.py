@@ -302,3 +302,25 @@ def test_tables_are_not_made_of_other_tensors():
     assert overlap(32, step_dev=8192 + 1192) == 1 and overlap(8, step_dev=8192 + 296) == 1
     assert overlap(32, step_dev=8192 + 1200) == 0 and overlap(8, step_dev=8192 + 300) == 0
     assert overlap(32, step_dev=16384) == 0 and overlap(8, step_dev=16384) == 1
+
+
+def test_the_timed_calls_are_there():
+    """What perf/operators.py calls of gsr.optim exists, with the arguments that it passes."""
+    import ast
+    import inspect
+    import os
+
+    from gsr import optim
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "perf", "operators.py")
+    with open(path) as f:
+        tree = ast.parse(f.read())
+    found = set()
+    for call in ast.walk(tree):
+        if not isinstance(call, ast.Call) or not isinstance(call.func, ast.Attribute):
+            continue
+        of = call.func.value
+        if (isinstance(of, ast.Call) and getattr(of.func, "id", "") == "_optim") or getattr(of, "id", "") == "optim":
+            target = getattr(optim, call.func.attr)
+            inspect.signature(target).bind(*call.args, **{k.arg: 0 for k in call.keywords})
+            found.add(call.func.attr)
+    assert found == {"AdamW", "clip_grad_norm_", "moments8_rows"}
