@@ -106,6 +106,33 @@ def test_flat_ranges_are_the_whole_step(bits):
         assert torch.equal(a.exp_avg, b.exp_avg)
 
 
+def test_ranks_agree_bit_for_bit(tmp_path):
+    """Two processes that exchange their gradients step the 8-bit buffer to the same bytes, whatever slices each
+    takes, and to those of one process that adds the two gradients itself."""
+    import os
+    import socket
+    import subprocess
+    import sys
+
+    import optim_rank_worker as worker
+    here = os.path.dirname(os.path.abspath(__file__))
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(
+        [os.path.join(os.path.dirname(here), "relightable3dgaussians-w_amd"), os.environ.get("PYTHONPATH", "")]))
+    ranks = [subprocess.Popen([sys.executable, os.path.join(here, "optim_rank_worker.py"), str(r), "2", str(port),
+                               str(tmp_path / "digest")], env=env) for r in range(2)]
+    try:
+        assert [p.wait(timeout=90) for p in ranks] == [0, 0]
+    finally:
+        for p in ranks:
+            p.kill()
+    digests = [(tmp_path / f"digest.{r}").read_text() for r in range(2)]
+    alone = worker.steps(2, lambda fp, step: worker.gradient(fp, step, 0) + worker.gradient(fp, step, 1), 1)
+    assert digests == [alone, alone]
+
+
 def test_a_plain_step_is_what_it_was():
     """Without decay and clipping the 32-bit step stays gsr_adam_step's."""
     a, b = flat(32), flat(32)
