@@ -354,21 +354,22 @@ __device__ __forceinline__ void adamw8_scalar(const AdamWTensor& t, const AdamWC
     }
 }
 
-// The largest of each L consecutive lanes, in all of them: rotations within rows of 16, then across
+// The largest of each L consecutive lanes, 32 or 64, in all of them: rotations within rows of 16, then across
 template <int L>
 __device__ __forceinline__ float lanes_max(float x) {
+    static_assert(L == 32 || L == 64, "at least two rows");
     x = fmaxf(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x128, 0xf, 0xf, true)));
     x = fmaxf(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x124, 0xf, 0xf, true)));
     x = fmaxf(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x122, 0xf, 0xf, true)));
     x = fmaxf(x, __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), 0x121, 0xf, 0xf, true)));
-    if (L >= 32) x = fmaxf(x, __shfl_xor(x, 16, 64));
-    if (L >= 64) x = fmaxf(x, __shfl_xor(x, 32, 64));
+    x = fmaxf(x, __shfl_xor(x, 16, 64));
+    if (L == 64) x = fmaxf(x, __shfl_xor(x, 32, 64));
     return x;
 }
 
 // Whole blocks: L = 64 / U lanes have one, lane l of them the four elements from 4 l of each of the
-// block's U parts.  A wave's loads are consecutive within its blocks, the blocks' maxima take four
-// to six exchanges, and each thread has 4 U elements in flight.
+// block's U parts.  A wave's loads are consecutive within its blocks, the blocks' maxima take five
+// or six exchanges, and each thread has 4 U elements in flight.
 template <int PT, int GT, int U>
 __device__ __forceinline__ void adamw8_vectors(const AdamWTensor& t, const AdamWConst& c, const AdamWScalars& s, float gs,
                                                long long lo) {
