@@ -241,11 +241,12 @@ def rasterize_gaussians_channels_backward(background, means3D, radii, feat, nch,
         keep = [_f32(x) for x in (background, means3D, scales, rotations, cov3D_precomp, viewmatrix, projmatrix,
                                   campos, dL_dout)]
         bg_, m_, sc_, rot_, cov_, vm_, pm_, cp_, dout_ = keep
+        radii_ = radii.contiguous()
         ptr = lambda t: t.data_ptr() if t.numel() else None
         ret = _lib.lib().gsr_backward_channels(
             P, int(nch), feat.size(1), _lib.fptr(feat), int(R), _lib.fptr(bg_), W, H, _lib.fptr(m_), _lib.fptr(sc_),
             float(scale_modifier), _lib.fptr(rot_), _lib.fptr(cov_), _lib.fptr(vm_), _lib.fptr(pm_), _lib.fptr(cp_),
-            float(tan_fovx), float(tan_fovy), radii.contiguous().data_ptr(), ptr(geomBuffer), ptr(binningBuffer),
+            float(tan_fovx), float(tan_fovy), radii_.data_ptr(), ptr(geomBuffer), ptr(binningBuffer),
             ptr(imageBuffer), _lib.fptr(dout_), dL_dmeans2D.data_ptr(), None, dL_dopacity.data_ptr(),
             dL_dfeat.data_ptr(), dL_dmeans3D.data_ptr(), ptr(dL_dcov3D), dL_dscales.data_ptr(),
             dL_drotations.data_ptr(), int(accumulate), _lib.stream_of(dev))

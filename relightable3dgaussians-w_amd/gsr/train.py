@@ -662,9 +662,10 @@ class _FusedViewRegs(torch.autograd.Function):
         dx = outs[0] if outs[0] is not None else (torch.empty(ctx.P, 3, device=scaling.device) if need[0] else None)
         ds = outs[1] if outs[1] is not None else (torch.empty_like(scaling) if need[1] else None)
         ptr = lambda t: None if t is None else t.data_ptr()
+        g = g.contiguous()  # held until the launch, as are all whose addresses it takes
         _lib.check(_lib.lib().gsr_view_regularisers_backward(ctx.P, ctx.V, scaling.data_ptr(), _lib.ptr_array(radii),
                                                              is_sky.data_ptr(), dcol.data_ptr(),
-                                                             g.contiguous().data_ptr(), ptr(dx), ptr(ds), acc,
+                                                             g.data_ptr(), ptr(dx), ptr(ds), acc,
                                                              _lib.stream_of(scaling.device)),
                    "gsr_view_regularisers_backward")
         if sk is not None:
@@ -710,8 +711,9 @@ class _RegsTail(torch.autograd.Function):
         V = s_.shape[0]
         d_sums = torch.empty_like(s_)
         d_env = torch.empty_like(e_)
+        g = g.float().contiguous()
         _lib.check(_lib.lib().gsr_view_regularisers_tail_backward(
-            V, ctx.ns, s_.data_ptr(), b_.data_ptr(), e_.data_ptr(), *ctx.consts, g.float().contiguous().data_ptr(),
+            V, ctx.ns, s_.data_ptr(), b_.data_ptr(), e_.data_ptr(), *ctx.consts, g.data_ptr(),
             d_sums.data_ptr(), d_env.data_ptr(), _lib.stream_of(s_.device)), "gsr_view_regularisers_tail_backward")
         return d_sums, d_env.view(ctx.env_shape), None, None, None
 
@@ -895,7 +897,8 @@ class _FusedSkyXYZ(torch.autograd.Function):
         L = _lib.lib()
         da = torch.empty_like(angles)
         dr = torch.empty(L.gsr_sky_xyz_partials(N), device=angles.device)
-        _lib.check(L.gsr_sky_xyz_backward(N, angles.data_ptr(), radius.data_ptr(), g.contiguous().data_ptr(),
+        g = g.contiguous()
+        _lib.check(L.gsr_sky_xyz_backward(N, angles.data_ptr(), radius.data_ptr(), g.data_ptr(),
                                           da.data_ptr(), dr.data_ptr(), _lib.stream_of(angles.device)),
                    "gsr_sky_xyz_backward")
         return da, dr.sum().reshape(radius.shape), None
