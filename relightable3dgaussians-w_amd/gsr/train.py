@@ -846,7 +846,8 @@ class _Activations(torch.autograd.Function):
         ctx.scene = scene
         ctx.box = box  # [GradSink]: set by model_fused once the outputs exist
         ctx.ins = ins
-        ctx.outs = (scale, rot, op, alb, rough, metal)
+        # (outputs as attributes would hold the node that they hold, and nothing would free either)
+        ctx.save_for_backward(scale, rot, op, alb, rough, metal)
         ctx.set_materialize_grads(False)
         return xyz, scale, rot, op, alb, rough, metal
 
@@ -856,6 +857,7 @@ class _Activations(torch.autograd.Function):
         lay, fp = scene.layout, scene.fp
         P, Nfg, Nsky = lay.P, lay.n_fg, lay.n_sky
         dev = ctx.ins[0].device
+        outs = ctx.saved_tensors
         ptr = lambda t: None if t is None or t.numel() == 0 else t.data_ptr()
         gs = [None if t is None else t.float().contiguous() for t in g]
         sk = ctx.box[0]
@@ -869,7 +871,7 @@ class _Activations(torch.autograd.Function):
         part = torch.empty(max(1, _lib.lib().gsr_activations_partials(P, Nfg)), dtype=torch.float32, device=dev)
         src = None if lay.src is None else lay.src.data_ptr()
         _lib.check(_lib.lib().gsr_activations_backward(
-            P, Nfg, Nsky, src, *[ptr(t) for t in ctx.ins], *[ptr(t) for t in ctx.outs], *[ptr(t) for t in gs],
+            P, Nfg, Nsky, src, *[ptr(t) for t in ctx.ins], *[ptr(t) for t in outs], *[ptr(t) for t in gs],
             ptr(d["xyz"]), ptr(d["sky_angles"]), ptr(d["sky_radius"]), part.data_ptr(), ptr(d["scaling"]),
             ptr(d["rotation"]), ptr(d["opacity"]), ptr(d["albedo"]), ptr(d["roughness"]), ptr(d["metalness"]),
             _lib.stream_of(dev)), "gsr_activations_backward")

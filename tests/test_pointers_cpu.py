@@ -76,3 +76,29 @@ def test_channels_backward(library):
         torch.zeros(4), torch.ones(P, 3), radii, torch.ones(P, 4), 4, torch.ones(P, 3), torch.ones(P, 4), 1.0, e,
         torch.eye(4), torch.eye(4), 1.0, 1.0, spread(4, H, W), torch.zeros(3), e, 0, e, e)
     assert library.calls == ["gsr_backward_channels"]
+
+
+def test_a_step_of_activations_leaves_nothing_behind(library):
+    """The activated tensors, and the buffers that collect their gradients, go when a training iteration lets go of
+    them: outputs that their own graph node holds as plain attributes would stay for good."""
+    import gc
+
+    from gsr import train
+    layout = types.SimpleNamespace(P=6, n_fg=4, n_sky=2, src=None)
+    p = {"xyz": (4, 3), "sky_angles": (2, 2), "sky_radius": (1,), "scaling": (6, 3), "rotation": (6, 4), "opacity": (6, 1),
+         "albedo": (4, 3), "roughness": (4, 1), "metalness": (4, 1)}
+    p = {k: torch.ones(shape, requires_grad=True) for k, shape in p.items()}
+    for t in p.values():
+        t.grad = torch.zeros_like(t)
+    scene = types.SimpleNamespace(layout=layout, sky_center=torch.zeros(3), fp=types.SimpleNamespace(params=p), is_sky=None)
+    for backward in (False, True):
+        model = train.RelitScene.model_fused(scene)
+        kept = [weakref.ref(t) for t in vars(model).values() if t is not None]
+        sink = model.get_xyz._gsr_sink[0]
+        kept += [weakref.ref(t) for t in sink.buf.values()] + [weakref.ref(sink)]
+        del sink
+        if backward:
+            sum(t.sum() for t in vars(model).values() if t is not None).backward()
+        del model
+        gc.collect()
+        assert [r() is None for r in kept] == [True] * len(kept)
