@@ -26,11 +26,12 @@
 // m / (sqrt(v) + eps) would be m / eps.
 //
 // Both steps are bound by HBM, at 28 and 16 bytes an element of an fp32 parameter (a copy in place
-// of 4 GB reaches 5.9 TB/s on the same card): 23.3M parameters 100 us (6.5 TB/s) and 67 us, 77.4M with
-// 8-bit moments 186 us (6.7 TB/s), 63.5M bf16 ones with masters 263 us (6.7 TB/s).  The 8-bit step's
+// of 4 GB reaches 5.9 TB/s on the same card).  Medians of a kernel trace: 23.3M parameters 100 us (6.5 TB/s)
+// and 73 us (5.1 TB/s; 62 us, 6.0 TB/s, where calls follow each other untraced), 77.4M with 8-bit moments
+// 189 us (6.6 TB/s), 63.5M bf16 ones with masters 262 us (6.8 TB/s).  The 8-bit step's
 // two roundings and their hash are about 60 vector instructions an element, which the loads in
 // flight of seven waves a SIMD still hide.  Small lists are bound by one launch's latency: 148 K
-// elements in 13 tensors 3.6 and 5.3 us.
+// elements in 13 tensors 3.8 and 5.4 us.
 #include "gsr_adamw.hpp"
 
 namespace gsr {
@@ -682,8 +683,10 @@ __device__ __forceinline__ void store_block(unsigned char* avg, unsigned char* r
 // An out block of 256 elements to a wave, four consecutive ones to a lane.  Divisions by cols
 // are products: with (2^64 - 1) / cols + 1 once a wave (exact while the dividend times cols is below
 // 2^64), and for what is left, below cols + 256, with ceil(2^20 / cols), or one comparison (cols >= 256).
-// Bound by its instructions (the vector units are 86 % busy): 23.2M elements of rows of 1 to 4, 164 MB,
-// 41 us (a copy's rate would be 28).  Eight blocks a wave, one after another, 65 against 51 us then; two
+// Bound by its instructions for the most part: 23.2M elements of rows of 1 to 4, 164 MB, take 41 us (a
+// copy's rate would be 28) and 18.8M vector instructions, about 27 us of that: an addition, product, mask
+// or move issues in 1.0 ns a SIMD here, a shift, select, comparison, maximum or conversion, six in ten of
+// them, in 1.75.  Eight blocks a wave, one after another, 65 against 51 us then; two
 // at once 57 against 55.
 __global__ void __launch_bounds__(256) k_moment_rows(MomentRowsTable a) {
     const int k = find_tensor<MR_TENSORS>(a.first, a.count, blockIdx.x);
@@ -934,7 +937,7 @@ __device__ __forceinline__ double squares_of(const AdamWTensor& t, u32 group) {
 }
 
 // Four groups a workgroup, the last ones first: 77.4M fp32 gradients between two steps 81 us, from the
-// first 95 (the step 186 us after either).  With loads past the caches 47 us, but the last step's stores
+// first 95 (the step takes as long after either).  With loads past the caches 47 us, but the last step's stores
 // are then written out during this one: 230 us, and 63.5M bf16 ones 37 + 322 against 53 + 261 us.
 template <int U>
 __global__ void __launch_bounds__(256) k_adamw_squares(AdamWTable a, u32 groups, double* __restrict__ partial) {
