@@ -812,9 +812,13 @@ class AdamW(torch.optim.Optimizer):
             states[k]["step"] = st["step"]
         for p in old:
             self.state.pop(p, None)
+        left = self._left_behind()
         for k, (p, q) in enumerate(zip(old, new)):
             g, at = where[id(p)]
             g["params"][at] = q
+            left.pop(p, None)
             if k in states:
                 self.state[q] = states[k]
+                if "master" in states[k]:
+                    left[q] = (q.data_ptr(), q._version)
         self._plans = None

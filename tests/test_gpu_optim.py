@@ -1175,6 +1175,30 @@ def test_replace_rows(optim, bits, kind):
     opt.step()
 
 
+def test_what_is_written_into_replaced_rows_is_kept(optim):
+    """A 16-bit parameter that replace_rows put in place and the program then writes: the step starts from that; kept
+    rows that it leaves alone have their masters' lower bits."""
+    opt, params, _ = make(optim, [(100, 3), (20,)], "bf16", weight_decay=0.0)
+    opt.step()
+    for same in (False, True):
+        p = opt.param_groups[0]["params"][0]
+        ix = torch.arange(100, device=DEV).flip(0)
+        master = opt.state[p]["master"][ix].clone()
+        q = p if same else p.detach()[ix].clone()
+        with torch.no_grad():
+            if same:
+                q.copy_(p[ix])
+        q.grad = torch.zeros_like(q)
+        opt.replace_rows([p], [q], [ix])
+        with torch.no_grad():
+            q[:50] = 3.0
+        st = opt.state[q]
+        st["exp_avg"].zero_()  # a step that moves nothing
+        opt.step()
+        want = torch.where(torch.arange(100, device=DEV).view(-1, 1) < 50, 3.0, master)
+        assert torch.equal(st["master"], want) and torch.equal(q.float(), want.to(q.dtype).float())
+
+
 def test_replace_rows_takes_each_parameter_once(optim):
     """A new parameter that is listed twice, or is another one of the optimizer's, is refused and nothing changes."""
     opt, params, _ = make(optim, [(10, 3), (10, 3)])
