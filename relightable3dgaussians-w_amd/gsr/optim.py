@@ -145,7 +145,8 @@ def moments8_encode(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor) -> Moments8
 
 
 def moments8_decode(moments: Sequence[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(exp_avg, exp_avg_sq) in 32 bits of 8-bit moments."""
+    """(exp_avg, exp_avg_sq) in 32 bits of 8-bit moments (infinity where a root's square is beyond
+    them, from 2^64 on)."""
     m = _check_moments8(moments, "moments")
     a, b = (torch.empty(m.exp_avg.shape, device=m.exp_avg.device) for _ in range(2))
     with _on(a.device):
